@@ -2986,7 +2986,7 @@ GEMM_FLOAT8_FEW_BYTES = 150e6
 # 128 columns that a wave has (8 waves); beyond 4,096 columns that is more than a launch in front.
 GEMM_FLOAT8_INLINE_ROWS = 16
 GEMM_FLOAT8_INLINE_COLUMNS = 4096
-GEMM_FLOAT8_SUMS_COLUMNS = 1024  # from here on gated rows in 8 bits may come of sums
+GEMM_FLOAT8_SUMS_COLUMNS = 1024  # from here on gated rows in 8 bits of many rows may come of sums (a second launch is longer than the few blocks of a tile)
 _E4M3, _E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 
 
@@ -3296,14 +3296,11 @@ def _float8_product(out, x, w: Float8, bias, swiglu: bool, limit, gelu: bool, se
     few = m <= GEMM_FLOAT8_INLINE_ROWS * groups if grouped else m <= GEMM_FLOAT8_FEW_ROWS and (m <= 16 or n * columns < GEMM_FLOAT8_FEW_BYTES)
     last = None  # what makes rows in 8 bits of sums
     if few and cs is not None:
-        # (the scale of a block waits for 128 units, a workgroup has few of them: units as a step of their own, from sums in 32-bit.  8 x 22016 x 4096 24
-        # microseconds, in tiles 47; K below GEMM_FLOAT8_SUMS_COLUMNS is a few blocks of a tile, and a second launch is longer)
-        if columns >= GEMM_FLOAT8_SUMS_COLUMNS:
-            ldc = 4 * -(-n // 4)
-            c, epilogue, n_out = torch.empty((m, ldc), dtype=torch.float32, device=rows.device), 1, n
-            last = segments[0].data_ptr() + 4 * groups if grouped else None, 1, 0
-        else:
-            few = False
+        # (the scale of a block waits for 128 units, a workgroup has few of them: units as a step of their own, from sums in 32-bit of exact
+        # products.  8 x 22016 x 4096 24 microseconds, in tiles 47)
+        ldc = 4 * -(-n // 4)
+        c, epilogue, n_out = torch.empty((m, ldc), dtype=torch.float32, device=rows.device), 1, n
+        last = segments[0].data_ptr() + 4 * groups if grouped else None, 1, 0
     inline, at_rows, at_xs, ldxs = False, rows.data_ptr(), None if xs is None else xs.data_ptr(), 0 if xs is None else xs.stride(0)
     if xs is None:
         inline = (few and rows.dtype is torch.bfloat16 and columns % 8 == 0 and ldx < 1 << 23 and at_rows % 16 == 0 and (m == 1 or ldx % 8 == 0)
@@ -3345,8 +3342,9 @@ def _float8_product(out, x, w: Float8, bias, swiglu: bool, limit, gelu: bool, se
 
 
 def gemm_float8(out, x, w: Float8, bias: torch.Tensor | None = None, *, swiglu: bool = False, limit: float | None = None, gelu: bool = False):
-    """The product of rows and a weight in 8 bits, sums in 32-bit over all of K, rounded once.  (Beyond 16 rows a bfloat16 or 8-bit result is that of
-    the matrix cores' 8-bit products, whose sums of 16 are off by up to 2^-13 of the largest product; a float32 result is not.)
+    """The product of rows and a weight in 8 bits, sums in 32-bit over all of K, rounded once.  (Beyond 16 rows a bfloat16 result, and beyond 64, or
+    16 of a weight of more than 150 MB, one in 8 bits, is that of the matrix cores' 8-bit products, whose sums of 16 are off by up to 2^-13 of the
+    largest product; a float32 result is not.  Of `grouped_float8` both are, beyond 16 rows a group in the mean.)
 
     x: `Float8` rows [M, K], or a bfloat16 or float32 matrix, which is taken to 8 bits as by rows_float8.
     plain:   out[M, N] = x w^T (+ bias, bfloat16), bfloat16 or float32.
