@@ -3243,7 +3243,7 @@ _FLOAT8_TILES = (((3, 256, 256), (4, 256, 192), (1, 128, 128), (0, 64, 64)), ((1
                  ((3, 256, 256), (1, 128, 128), (0, 64, 64)), ((3, 256, 256), (2, 128, 256), (1, 128, 128), (0, 64, 64)))
 
 
-def _float8_product(out, x, w: Float8, bias, swiglu: bool, limit, gelu: bool, segments, what: str):
+def _float8_product(out, x, w: Float8, bias, swiglu: bool, limit, gelu: bool, exact: bool, segments, what: str):
     grouped = segments is not None
     if isinstance(x, Float8):
         _float8_rows(x, "x")
@@ -3294,6 +3294,9 @@ def _float8_product(out, x, w: Float8, bias, swiglu: bool, limit, gelu: bool, se
     if m == 0:
         return out
     few = m <= GEMM_FLOAT8_INLINE_ROWS * groups if grouped else m <= GEMM_FLOAT8_FEW_ROWS and (m <= 16 or n * columns < GEMM_FLOAT8_FEW_BYTES)
+    exact = bool(exact) and epilogue != 1  # (results in 32 bits always are)
+    if exact and not grouped and m > 16 and cs is None:
+        few = False  # (the stream's results in bfloat16 of more rows are of 8-bit products)
     last = None  # what makes rows in 8 bits of sums
     if few and cs is not None:
         # (the scale of a block waits for 128 units, a workgroup has few of them: units as a step of their own, from sums in 32-bit of exact
@@ -3329,33 +3332,35 @@ def _float8_product(out, x, w: Float8, bias, swiglu: bool, limit, gelu: bool, se
         return out if last is None else _units_of_sums(out, c, n_out // 2, unit, limit, what, index, *last)
     kp, sums = w.values.shape[-1], None
     if grouped:
-        tile, each = 1 if cs is None else 2, kp // FLOAT8_BLOCK
+        tile, each, end = 1 if cs is None or exact else 2, kp // FLOAT8_BLOCK, segments[0].data_ptr() + 4 * groups
     else:
-        tile, each = gemm_float8_tiles(m, n, columns, epilogue, _cus(index))
-        if each * FLOAT8_BLOCK < kp or (cs is not None and tile < 2):
-            sums = torch.empty((-(-kp // (each * FLOAT8_BLOCK)), m, 4 * -(-n // 4)), dtype=torch.float32, device=rows.device)
+        (tile, each), end = gemm_float8_tiles(m, n, columns, 1 if exact else epilogue, _cus(index)), None
+    if exact or each * FLOAT8_BLOCK < kp or (cs is not None and tile < 2):
+        sums = torch.empty((-(-kp // (each * FLOAT8_BLOCK)), m, 4 * -(-n // 4)), dtype=torch.float32, device=rows.device)
     in_sums = cs is not None and sums is not None  # (units as a step of their own)
-    _launch(index, what, _entry("gemm_float8", "llms_gemm_float8", "iiplpiplpippipiiiifppillip"), tile, 4 if in_sums else epilogue, c.data_ptr(), ldc,
+    _launch(index, what, _entry("gemm_float8", "llms_gemm_float8", "iiplpiplpippipiiiifppilliip"), tile, 4 if in_sums else epilogue, c.data_ptr(), ldc,
             0 if cs is None else cs.data_ptr(), 0 if cs is None else cs.stride(0), at_rows, *common, kp, unit, limit or 0.0,
-            seg, tile_start, groups, w_stride, ws_stride, each, None if sums is None else sums.data_ptr())
-    return _units_of_sums(out, sums, n_out, unit, limit, what, index, None, sums.shape[0], sums.stride(0)) if in_sums else out
+            seg, tile_start, groups, w_stride, ws_stride, each, exact, None if sums is None else sums.data_ptr())
+    return _units_of_sums(out, sums, n_out, unit, limit, what, index, end, sums.shape[0], sums.stride(0)) if in_sums else out
 
 
-def gemm_float8(out, x, w: Float8, bias: torch.Tensor | None = None, *, swiglu: bool = False, limit: float | None = None, gelu: bool = False):
+def gemm_float8(out, x, w: Float8, bias: torch.Tensor | None = None, *, swiglu: bool = False, limit: float | None = None, gelu: bool = False,
+                exact: bool = False):
     """The product of rows and a weight in 8 bits, sums in 32-bit over all of K, rounded once.  (Beyond 16 rows a bfloat16 result, and beyond 64, or
     16 of a weight of more than 150 MB, one in 8 bits, is that of the matrix cores' 8-bit products, whose sums of 16 are off by up to 2^-13 of the
-    largest product; a float32 result is not.  Of `grouped_float8` both are, beyond 16 rows a group in the mean.)
+    largest product; a float32 result is not.  Of `grouped_float8` both are, beyond 16 rows a group in the mean.  With `exact` none is: sums of exact
+    products, which leave in float32 and are rounded by a launch behind: 2048 x 12288 x 4096 takes 218 microseconds and not 91, 64 rows 22 and not 19.)
 
     x: `Float8` rows [M, K], or a bfloat16 or float32 matrix, which is taken to 8 bits as by rows_float8.
     plain:   out[M, N] = x w^T (+ bias, bfloat16), bfloat16 or float32.
     swiglu:  w = [gate; up] ([2I, K]): out[M, I] = silu(gate) * up, or with `limit` or `gelu` the units of `silu_mul`, in 32-bit; out is
              bfloat16, or a `Float8` (rows in 8 bits for the next product)."""
-    return _float8_product(out, x, w, bias, swiglu, limit, gelu, None, "gemm_float8")
+    return _float8_product(out, x, w, bias, swiglu, limit, gelu, exact, None, "gemm_float8")
 
 
 def grouped_float8(out, x, w: Float8, segments: "tuple[torch.Tensor, torch.Tensor]", *, swiglu: bool = False, limit: float | None = None,
-                   gelu: bool = False):
+                   gelu: bool = False, exact: bool = False):
     """gemm_float8 with a weight per segment of rows: w [G, N, K], `segments` = (seg [G + 1], tile_start [2, G + 1]) on the device (what
     `moe_sort` returns), rows seg[g] .. seg[g + 1] of x and out belonging to group g.  seg starts with 0, does not fall and ends at or
     before the last row; rows of out behind its end are left as they are."""
-    return _float8_product(out, x, w, None, swiglu, limit, gelu, segments, "grouped_float8")
+    return _float8_product(out, x, w, None, swiglu, limit, gelu, exact, segments, "grouped_float8")

@@ -80,3 +80,111 @@ def test_units_of_few_rows_per_group_in_8_bits_are_of_exact_sums(counts, inter, 
     pairs_of = [sums_of(xd[i: i + 1], wd[g]) for i, g in enumerate(group.tolist())]
     want, off = units_of(*(torch.cat(t) for t in zip(*pairs_of)), inter)
     check_steps(out, want, off)
+
+
+def check_bfloat16(out, want, off):
+    """Results between the roundings of want - off and want + off."""
+    low, high = ((want + d).to(torch.bfloat16).double() for d in (-off, off))  # (rounding keeps the order)
+    got = out.cpu().double()
+    wrong = ((got < low) | (got > high)).sum().item()
+    assert wrong == 0, f"{wrong} of {got.numel()} values are not the rounding of any number that 32-bit sums allow"
+
+
+@pytest.mark.parametrize("m,inter,k", [(1, 64, 300), (20, 130, 85), (64, 70, 600), (65, 129, 512), (130, 200, 96), (300, 257, 700), (200, 90, 4500)])
+def test_exact_sums(m, inter, k):
+    """Asked for, at any number of rows: plain with a bias, gated, gated to 8 bits."""
+    n = 2 * inter
+    x8, w8, xd, (wd,) = operands(m, n, k, m + inter + k)
+    y, off = sums_of(xd, wd)
+    want, carried = units_of(y, off, inter)
+    bias = torch.randn(n, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    yb = y + bias.double()
+    out = torch.full((m + 1, n + 3), float("nan"), dtype=torch.bfloat16, device=DEV)
+    ops().gemm_float8(out[:m, :n], x8, w8, bias.to(DEV), exact=True)
+    check_bfloat16(out[:m, :n], yb, off + (yb.abs() + off) * 2.0 ** -23)
+    assert torch.isnan(out[m:]).all() and torch.isnan(out[:, n:]).all()
+    out = torch.full((m + 1, inter + 3), float("nan"), dtype=torch.bfloat16, device=DEV)
+    ops().gemm_float8(out[:m, :inter], x8, w8, swiglu=True, exact=True)
+    check_bfloat16(out[:m, :inter], want, carried)
+    assert torch.isnan(out[m:]).all() and torch.isnan(out[:, inter:]).all()
+    check_steps(ops().gemm_float8(ops().empty_float8(m, inter, DEV), x8, w8, swiglu=True, exact=True), want, carried)
+    # a float32 result is exact anyhow
+    a, b = (ops().gemm_float8(torch.empty(m, n, device=DEV), x8, w8, exact=e) for e in (False, True))
+    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("tile,each", [(0, None), (0, 4), (1, None), (1, 4)])
+@pytest.mark.parametrize("m,inter,k", [(70, 45, 1300), (129, 258, 1030)])
+def test_exact_sums_of_every_tile_and_part(tile, each, m, inter, k, monkeypatch):
+    from llmserve.ops import library
+
+    monkeypatch.setattr(library, "gemm_float8_tiles", lambda *a: (tile, each or -(-k // 128)))
+    x8, w8, xd, (wd,) = operands(m, 2 * inter, k, m + inter + k)
+    y, off = sums_of(xd, wd)
+    want, carried = units_of(y, off, inter)
+    room = lambda cols: torch.empty(m, cols, dtype=torch.bfloat16, device=DEV)  # noqa: E731
+    check_bfloat16(ops().gemm_float8(room(2 * inter), x8, w8, exact=True), y, off)
+    check_bfloat16(ops().gemm_float8(room(inter), x8, w8, swiglu=True, exact=True), want, carried)
+    check_steps(ops().gemm_float8(ops().empty_float8(m, inter, DEV), x8, w8, swiglu=True, exact=True), want, carried)
+
+
+@pytest.mark.parametrize("counts", [[3, 0, 9], [40, 0, 129, 300, 1], [0, 0, 128, 0, 256]])
+@pytest.mark.parametrize("inter,k", [(65, 200), (136, 640)])
+def test_exact_sums_of_groups(counts, inter, k):
+    """Rows behind the last segment are left as they are."""
+    pairs, groups, n = sum(counts), len(counts), 2 * inter
+    x8, w8, xd, wd = operands(pairs + 2, n, k, pairs + k, groups)
+    group = torch.repeat_interleave(torch.arange(groups), torch.tensor(counts))
+    segments = segments_of(counts)
+    y, off = torch.zeros(pairs, n, dtype=torch.float64), torch.zeros(pairs, n, dtype=torch.float64)
+    for g in set(group.tolist()):
+        y[group == g], off[group == g] = sums_of(xd[:pairs][group == g], wd[g])
+    want, carried = units_of(y, off, inter)
+    for cols, swiglu, expected, slack in ((n, False, y, off), (inter, True, want, carried)):
+        out = torch.full((pairs + 2, cols + 1), float("nan"), dtype=torch.bfloat16, device=DEV)
+        ops().grouped_float8(out[:, :cols], x8, w8, segments, swiglu=swiglu, exact=True)
+        check_bfloat16(out[:pairs, :cols], expected, slack)
+        assert torch.isnan(out[pairs:]).all() and torch.isnan(out[:, cols:]).all()
+    out8 = ops().empty_float8(pairs + 2, inter, DEV)
+    out8.values.view(torch.uint8).fill_(7)
+    out8.scale.view(torch.uint8).fill_(9)
+    ops().grouped_float8(out8, x8, w8, segments, swiglu=True, exact=True)
+    check_steps(ops().Float8(out8.values[:pairs], out8.scale[:pairs], inter), want, carried)
+    assert (out8.values.view(torch.uint8)[pairs:] == 7).all() and (out8.scale.view(torch.uint8)[pairs:] == 9).all()
+    a, b = (ops().grouped_float8(torch.zeros(pairs + 2, n, device=DEV), x8, w8, segments, exact=e) for e in (False, True))
+    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("kind", ["plain", "gated", "rows"])
+def test_exact_sums_in_two_graphs(kind):
+    """Two graphs of one call in turn, with other rows each time: the sums' place is a call's own."""
+    m, n, k = 90, 406, 700
+    w8 = ops().weight_float8((torch.randn(n, k, generator=torch.Generator().manual_seed(n)) * k ** -0.5).to(torch.bfloat16).to(DEV))
+
+    def room():
+        return ops().empty_float8(m, n // 2, DEV) if kind == "rows" else torch.empty(m, n if kind == "plain" else n // 2, dtype=torch.bfloat16, device=DEV)
+
+    def call(out, x):
+        return ops().gemm_float8(out, x, w8, swiglu=kind != "plain", exact=True)
+
+    def bytes_of(out):
+        return [t.clone().view(torch.uint8) for t in (out[:2] if kind == "rows" else (out,))]
+
+    xs, outs, graphs = [torch.empty(m, k, dtype=torch.bfloat16, device=DEV) for _ in range(2)], [room(), room()], []
+    for x, out in zip(xs, outs):
+        x.normal_()
+        call(out, x)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            call(out, x)
+        graphs.append(graph)
+    for turn in range(4):
+        for x in xs:
+            x.normal_()
+        wanted = [bytes_of(call(room(), x)) for x in xs]
+        for graph in graphs if turn % 2 else graphs[::-1]:
+            graph.replay()
+        torch.cuda.synchronize()
+        for out, want in zip(outs, wanted):
+            assert all(torch.equal(a, b) for a, b in zip(bytes_of(out), want))
