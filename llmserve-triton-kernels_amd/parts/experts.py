@@ -173,9 +173,8 @@ class Experts(FeedForward):
         return results
 
     def _products_float8(self, x, segments):
-        """The same with weights in 8 bits; what goes from the first product to the second is in 8 bits where the rows are many."""
+        """The same with weights in 8 bits; what goes from the first product to the second is rounded once, to 8 bits, however many the rows."""
         pairs, dev = x.shape[0], x.device
-        few = pairs <= ops.GEMM_FLOAT8_INLINE_ROWS * self.experts
-        act = torch.empty((pairs, self.intermediate), dtype=torch.bfloat16, device=dev) if few else ops.empty_float8(pairs, self.intermediate, dev)
+        act = ops.empty_float8(pairs, self.intermediate, dev)
         ops.grouped_float8(act, x, self.w_gate_up, segments, swiglu=True, limit=self.limit if self.unit == "clamped" else None)
         return ops.grouped_float8(torch.empty((pairs, self.hidden), dtype=torch.float32, device=dev), act, self.w_down, segments)

@@ -8,7 +8,7 @@ ops.gemm_stream, ops.gemm_tiles), and in 32-bit with up to 16 rows and SiLU (ops
 library, more 32-bit rows, and sizes those kernels do not take have the activation as a kernel of its own.
 
 With weights in 8 bits (the engine's weights="float8") both products are ops.gemm_float8's; the first one's result is rounded once, to 8 bits, and that is
-what the second one multiplies, but for the rows of `_units_in_bfloat16`."""
+what the second one multiplies."""
 
 from __future__ import annotations
 
@@ -65,19 +65,10 @@ class SwiGLU(FeedForward):
 
     adds_to_stream_by = "down"
 
-    def _units_in_bfloat16(self, m: int) -> bool:
-        """Where the first product's units, which are in its epilogue then, are rounded to bfloat16 and become 8 bits in the second one.  Up to 16 short rows: inside
-        it.  33 to 64 rows: by a launch in front of it, as in 8 bits they would be a step of their own, from sums twice as wide in 32-bit (64 x 22016 x 4096
-        33 and 37 microseconds with that launch, 32 rows the same, 8 rows 25.3 and 24.5)."""
-        short = m <= ops.GEMM_FLOAT8_INLINE_ROWS and self.intermediate <= ops.GEMM_FLOAT8_INLINE_COLUMNS
-        return short or 32 < m <= ops.GEMM_FLOAT8_FEW_ROWS
-
     def _forward_float8(self, x):
         rows = normed_float8(x) if isinstance(x, DeferredNorm) else x
         values = rows.values if isinstance(rows, ops.Float8) else rows
-        m, device = values.shape[0], values.device
-        act = (torch.empty((m, self.intermediate), dtype=torch.bfloat16, device=device) if self._units_in_bfloat16(m)
-               else ops.empty_float8(m, self.intermediate, device))
+        act = ops.empty_float8(values.shape[0], self.intermediate, values.device)  # (whatever the rows: in bfloat16 first they would be rounded twice)
         ops.gemm_float8(act, rows, self.gate_up, swiglu=True, limit=self.limit, gelu=self.gelu)
         return linear(act, self.down, out_dtype=self.result_dtype)
 

@@ -188,3 +188,16 @@ def test_exact_sums_in_two_graphs(kind):
         torch.cuda.synchronize()
         for out, want in zip(outs, wanted):
             assert all(torch.equal(a, b) for a, b in zip(bytes_of(out), want))
+
+
+@pytest.mark.parametrize("inter,k", [(176, 640), (129, 3000)])
+def test_units_in_8_bits_of_a_row_are_the_same_beside_any_others(inter, k):
+    """Of up to 64 rows (K in one part, up to 4,096 columns): the same sums in the same order, whichever rows come with it, so a step may be filled up."""
+    x8, w8, _, _ = operands(64, 2 * inter, k, inter)
+    outs = {}
+    for m in (1, 2, 15, 16, 17, 31, 32, 33, 63, 64):
+        rows = ops().Float8(x8.values[:m], x8.scale[:m], k)
+        outs[m] = ops().gemm_float8(ops().empty_float8(m, inter, DEV), rows, w8, swiglu=True)
+    for m, out in outs.items():
+        assert torch.equal(out.values.view(torch.uint8), outs[64].values[:m].view(torch.uint8)), m
+        assert torch.equal(out.scale.view(torch.uint8), outs[64].scale[:m].view(torch.uint8)), m
