@@ -31,7 +31,8 @@ def main(argv=None) -> int:
     ap.add_argument("--device", default="cuda", help="GPU to run on (there is no CPU path)")
     ap.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
     ap.add_argument("--weights", choices=["model", "float8"], default="model",
-                    help="float8: hold the layers' matrices, and multiply their rows, in 8-bit floating point")
+                    help="float8: hold the matrices of plain attention, gated feed-forwards and experts, and multiply their rows, in 8-bit "
+                         "floating point (a model's other parts keep theirs, with a warning)")
     ap.add_argument("--random-weights", action="store_true", help="--model names a size; fill it from --seed")
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--block-size", type=int, default=16)

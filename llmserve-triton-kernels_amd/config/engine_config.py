@@ -29,8 +29,9 @@ class EngineConfig:
     # replay steps from captured HIP graphs: decode-only steps, and steps with portions of prompts that are small
     # enough for the host's launches to be their limit (a rule by sizes; a bucket of sizes is captured at its second use)
     use_graphs: bool = True
-    # "float8": attention's and the feed-forwards' matrices are held, and their products' rows multiplied, in 8-bit floating point with a
-    # power of two per block of 128 (made from the checkpoint's weights at load; embedding, head and everything else stay in `dtype`)
+    # "float8": the matrices of softmax attention without additions (the part "attention"), of gated feed-forwards ("swiglu") and of experts are held, and
+    # their products' rows multiplied, in 8-bit floating point with a power of two per block of 128 (made from the checkpoint's weights at load).
+    # Everything else stays in `dtype`: embedding, head, routers, ungated feed-forwards, and all other mixers; which ones a model has is warned of
     weights: str = "model"
 
     def validate(self) -> None:

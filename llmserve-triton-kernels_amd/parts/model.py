@@ -9,13 +9,15 @@ project only the rows whose logits are wanted.
 
 from __future__ import annotations
 
+import warnings
+
 import torch
 
 from ..ops import library as ops
 from . import (attention, attention_composed, attention_latent, block, connection, decay_attention, delta_rule, embedding,  # noqa: F401
                experts, gate, layernorm, rmsnorm, rope, selective_scan, side_by_side, state_space, swiglu, ungated)  # (register the built-in parts)
 from .registry import (BLOCKS, CONNECTIONS, EMBEDDINGS, FEED_FORWARDS, GATES, HEADS, MIXERS, NORMS, BuildContext, DeferredNorm,
-                       OpenStreams, Part)
+                       FeedForward, Mixer, OpenStreams, Part)
 from .spec import ModelSpec, ParamInfo
 
 
@@ -41,8 +43,12 @@ class Model:
                                  f"the spec names parts for {sorted(layer.parts)} and weights for {sorted(layer.weights)}")
             self.blocks.append(block({role: families[family].build(layer.parts[role], ctx)
                                       for role, family in block.ROLES.items()}))
-        if ctx.weights == "float8" and not any(part.takes_float8_weights for _, part in self._parts()):
-            raise ValueError("no part of this model holds weights in 8 bits")
+        if ctx.weights == "float8":
+            held, kept = self.float8_parts()
+            if not held:
+                raise ValueError("no part of this model holds weights in 8 bits")
+            if kept:
+                warnings.warn(f"weights='float8': 8 bits for the matrices of {', '.join(held)}; those of {', '.join(kept)} stay in {str(ctx.dtype).removeprefix('torch.')}", stacklevel=2)
 
     # ---- tensors -------------------------------------------------------------------------
     def _parts(self) -> list[tuple[str, Part]]:
@@ -52,6 +58,16 @@ class Model:
         for layer, blk in zip(self.spec.layers, self.blocks):
             out += [(layer.weights[role], part) for role, part in blk.parts.items()]
         return out
+
+    def float8_parts(self) -> tuple[list[str], list[str]]:
+        """The kinds of mixers and feed-forwards with matrices that hold them in 8 bits where weights are to be, and of those that do not."""
+        held, kept = {}, {}
+        for blk in self.blocks:
+            for part in blk.parts.values():
+                for one in getattr(part, "members", [part]):
+                    if isinstance(one, (Mixer, FeedForward)) and any(len(info.shape) > 1 for info in one.param_infos().values()):
+                        (held if one.takes_float8_weights else kept)[one.spec.kind] = None
+        return list(held), list(kept)
 
     def param_infos(self) -> dict[str, ParamInfo]:
         """Every tensor of the checkpoint by its name."""

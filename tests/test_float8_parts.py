@@ -54,3 +54,60 @@ def test_units_of_experts_are_rounded_once_whatever_the_rows(products, pairs):
     part._products_float8(torch.zeros(pairs, 64, dtype=BF16), None)
     (_, act), (x, _) = products
     assert isinstance(act, ops.Float8) and x is act and act.columns == 100
+
+
+# What each family's mixers and feed-forwards do, and the 8-bit matrices that its parts hold once loaded.
+FAMILIES = {
+    "tiny-a": (["attention", "swiglu"], []),
+    "dibepel-tiny": (["swiglu"], ["composed_attention"]),
+    "milozen-tiny": (["swiglu", "experts"], ["latent_attention"]),
+    "felavik-tiny": (["experts"], ["composed_attention", "decay_attention"]),
+    "nolavik-tiny": (["experts"], ["composed_attention", "gated_delta", "latent_attention", "selective_scan"]),
+    "zotunex-tiny": (["experts"], ["composed_attention", "latent_attention", "ungated"]),
+    "ramolix-tiny": (["swiglu"], ["composed_attention", "latent_attention", "state_space"]),
+}
+HELD = {"attention": {"qkv_weight", "o_weight"}, "swiglu": {"gate_up", "down"}, "experts": {"w_gate_up", "w_down"}}
+
+
+@pytest.mark.parametrize("name", FAMILIES)
+def test_which_matrices_a_family_holds_in_8_bits(name, products):
+    """And a warning names the parts that keep theirs."""
+    import warnings
+
+    from llmserve.config.registry import architecture_of, preset
+    from llmserve.parts.model import Model
+
+    config = preset(name)
+    arch = architecture_of(config)
+    held, kept = FAMILIES[name]
+    with warnings.catch_warnings(record=True) as seen:
+        warnings.simplefilter("always")
+        model = Model(arch.build_spec(arch.config_class.from_dict(config)), BuildContext(BF16, CPU, "float8"))
+    got = model.float8_parts()
+    assert set(got[0]) == set(held) and set(got[1]) == set(kept)
+    assert len(seen) == (1 if kept else 0)
+    for kind in kept:
+        assert kind in str(seen[0].message)
+    model.load({name: torch.zeros(info.shape, dtype=BF16) for name, info in model.param_infos().items()})
+    holders = set()
+    for _, part in model._parts():
+        for one in (part, *getattr(part, "members", ()), getattr(part, "shared_unit", None)):
+            if one is None:
+                continue
+            in_8_bits = {n for n, v in vars(one).items() if isinstance(v, ops.Float8)}
+            if in_8_bits:
+                assert in_8_bits == HELD[one.spec.kind]
+                holders.add(one.spec.kind)
+            else:
+                assert one.spec.kind not in HELD
+    assert set(held) <= holders <= set(held) | {"swiglu"}  # (the unit beside the experts is one)
+
+
+def test_a_model_in_its_own_type_is_not_warned_of(recwarn):
+    from llmserve.config.registry import architecture_of, preset
+    from llmserve.parts.model import Model
+
+    config = preset("ramolix-tiny")
+    arch = architecture_of(config)
+    Model(arch.build_spec(arch.config_class.from_dict(config)), BuildContext(BF16, CPU))
+    assert not len(recwarn)
