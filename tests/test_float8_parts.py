@@ -111,3 +111,28 @@ def test_a_model_in_its_own_type_is_not_warned_of(recwarn):
     arch = architecture_of(config)
     Model(arch.build_spec(arch.config_class.from_dict(config)), BuildContext(BF16, CPU))
     assert not len(recwarn)
+
+
+@pytest.mark.parametrize("flags,weights", [([], "model"), (["--weights", "model"], "model"), (["--weights", "float8"], "float8")])
+def test_the_command_line_hands_the_option_on(flags, weights, monkeypatch):
+    from llmserve import cli
+    from llmserve.engine import llm
+
+    class Seen(Exception):
+        pass
+
+    def made(model, *, engine, **options):
+        engine.validate()
+        raise Seen(engine.weights)
+
+    monkeypatch.setattr(llm, "LLM", made)
+    with pytest.raises(Seen, match=f"^{weights}$"):
+        cli.main(["--model", "tiny", *flags])
+
+
+def test_the_command_line_refuses_other_weights(capsys):
+    from llmserve import cli
+
+    with pytest.raises(SystemExit):
+        cli.main(["--model", "tiny", "--weights", "int4"])
+    assert "float8" in capsys.readouterr().err
