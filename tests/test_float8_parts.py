@@ -136,3 +136,12 @@ def test_the_command_line_refuses_other_weights(capsys):
     with pytest.raises(SystemExit):
         cli.main(["--model", "tiny", "--weights", "int4"])
     assert "float8" in capsys.readouterr().err
+
+
+@pytest.mark.parametrize("n,k", [((1 << 32) - (1 << 23), 128), (262144 - 512, 16384), (2, 1 << 23)])
+def test_weights_beyond_32_bit_offsets_are_refused(n, k):
+    n = n // 128 if k == 128 else n
+    w = ops.Float8(torch.empty((n, k), dtype=torch.float8_e4m3fn, device="meta"),
+                   torch.empty((-(-n // 128), ops.float8_scale_columns(k)), dtype=torch.float8_e8m0fnu, device="meta"), k)
+    with pytest.raises(ValueError, match="too large"):
+        ops.gemm_float8(torch.empty((1, n), dtype=torch.float32, device="meta"), torch.empty((1, k), dtype=BF16, device="meta"), w)
