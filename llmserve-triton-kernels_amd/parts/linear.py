@@ -311,8 +311,6 @@ def normed_float8(x):
 
 
 def _linear_float8(x, weight, bias, out_dtype, out):
-    if isinstance(x, JoinedRows):
-        x = x.materialize()
     m, device = (x.values if isinstance(x, ops.Float8) else x).shape[0], weight.values.device
     if out is None:
         out = torch.empty((m, weight.values.shape[0]), dtype=out_dtype or torch.bfloat16, device=device)
@@ -322,7 +320,8 @@ def _linear_float8(x, weight, bias, out_dtype, out):
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
            out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None, from_cache: bool = False) -> torch.Tensor:
     """x [M, K] (unit inner stride; or `JoinedRows`), weight [N, K] -> [M, N] in out_dtype (default: x's).  `from_cache`: as for
-    ops.gemm_tiles.  A weight in 8 bits takes rows in bfloat16 or in 8 bits, and out_dtype is bfloat16 if not given."""
+    ops.gemm_tiles.  A weight in 8 bits takes rows in bfloat16 or in 8 bits (and no `JoinedRows`: no part with such a weight accepts them), and
+    out_dtype is bfloat16 if not given."""
     if isinstance(weight, ops.Float8):
         return _linear_float8(x, weight, bias, out_dtype, out)
     out_dtype = out_dtype or x.dtype
