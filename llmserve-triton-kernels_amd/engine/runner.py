@@ -69,6 +69,7 @@ class ModelRunner:
         else:
             budget = engine_config.kv_bytes
             if budget is None:
+                torch.cuda.empty_cache()  # (what the checkpoint's tensors took while they were laid out, or became 8 bits, is free again)
                 free, _total = torch.cuda.mem_get_info(device)
                 budget = int(free * engine_config.gpu_memory_fraction)
             # the state of all slots comes off the budget; every paged group gets pages for the same number of longest
@@ -140,6 +141,7 @@ class ModelRunner:
         ops.ensure_built(engine_config.dtype, extra=model.libraries(engine_config.dtype))
         tensors = random_tensors(model.param_infos(), seed, dtype, device if on_device else "cpu")
         model.load({k: v.to(device) for k, v in tensors.items()})
+        del tensors  # (what no part has kept as it was is free before the cache is sized)
         return cls(model, config, engine_config, device)
 
     # ---- requests -------------------------------------------------------------------------
