@@ -71,9 +71,11 @@ __device__ __forceinline__ float f8_scale(uint32_t byte) { return __uint_as_floa
 
 __device__ __forceinline__ uint32_t f8_magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-// x / (1 + exp(-x)) in 32 bits, to a few units in the last place: the hardware's exp2 and reciprocal with one Newton step (an expf and
-// a division are some 35 instructions, these 9).  Numerator and denominator are a quarter of what they stand for, and bounded, so
-// that no reciprocal is a denormal number; x below -89 gives -0, NaN and -infinity NaN, as the formula does.
+// x / (1 + exp(-x)) of a 32-bit number, by the steps that common.h has for bfloat16 ones: the hardware's exp2 and reciprocal with one Newton step (an expf
+// and a division are some 35 instructions, these 9).  The exponent x log2(e) is rounded once, at its size, so the result is some 2 units of 2^-24 off for x
+// above 0, 9 down to -10, 30 down to -30 and 65 down to -88, where it is 2^-121: at most 4e-6 of it, beside the 2^-4 or 2^-8 of what it is rounded to
+// behind.  Numerator and denominator are a quarter of what they stand for, and bounded, so that no reciprocal is a denormal number; x
+// below -89 gives -0, NaN and -infinity NaN, as the formula does.
 __device__ __forceinline__ float f8_silu(float x) { return silu_of_bf16(x); }
 
 // gated units, in 32 bits: 0 SiLU, 1 clamped, 3 gelu (the numbers of the product kernels).  A NaN stays one, so it is no fminf that clamps.

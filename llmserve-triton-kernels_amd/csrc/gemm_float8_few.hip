@@ -1,13 +1,17 @@
-// The product of few rows in 8-bit floating point against a weight in 8 bits (gemm_float8.hip says which), up to 64 rows: decoding.
-// What bounds it is reading the weight.
+// Products of few rows in 8-bit floating point against weights in 8 bits (gemm_float8.hip says which): decoding.  What bounds them is reading the weight.
 //
-// A workgroup of 8 waves owns TN blocks of 16 weight rows and all (up to 16 TM) rows of X; its waves share K out in blocks of 128, wave w
+//   gemm_float8_stream   one weight and up to 64 rows: a workgroup a compute unit, with X in its registers; described where it begins
+//   gemm_float8_join     the sums of its parts of K
+//   gemm_float8_few      a weight per group of rows, of up to 16 in the mean; described here
+//
+// A workgroup of 8 waves owns TN blocks of 16 rows of a group's weight and walks the group's rows 16 at a time, reading the weight anew for each 16: groups
+// far above the mean take as many passes as they have sixteens, which stand behind one another.  Its waves share K out in blocks of 128, wave w
 // takes blocks w, w + 8, ..., and meet in LDS in the order of the waves.  Weights come straight from memory into the registers of the matrix
 // instruction: a lane takes the pieces g and g + 4 of 16 bytes of its row's 128 (g = lane / 16), so an instruction reads 64 bytes of
 // each of 16 rows in one piece, and X is read the same way.
 //
-// X in bfloat16 becomes 8 bits on the way in: a lane has 32 of the 128 numbers of its row, the block's largest is two exchanges between the
-// four lanes of the row away, and the conversion divides by the scale itself (v_cvt_scalef32_pk_fp8_bf16).  Every workgroup does that
+// X in bfloat16 becomes 8 bits on the way in (in the stream too): a lane has 32 of the 128 numbers of its row, the block's largest is two exchanges between
+// the four lanes of the row away, and the conversion divides by the scale itself (v_cvt_scalef32_pk_fp8_bf16).  Every workgroup does that
 // for itself: some 90 vector instructions per block of 128 columns and 16 rows, where another launch in front costs more.
 #include "float8.h"
 
