@@ -2,7 +2,7 @@
 //
 //   gemm_float8_stream   one weight and up to 64 rows: a workgroup a compute unit, with X in its registers; described where it begins
 //   gemm_float8_join     the sums of its parts of K
-//   gemm_float8_few      a weight per group of rows, of up to 16 in the mean; described here
+//   gemm_float8_few      a weight per group of rows, of up to 8 in the mean; described here
 //
 // A workgroup of 8 waves owns TN blocks of 16 rows of a group's weight and walks the group's rows 16 at a time, reading the weight anew for each 16: groups
 // far above the mean take as many passes as they have sixteens, which stand behind one another.  Its waves share K out in blocks of 128, wave w

@@ -2984,8 +2984,16 @@ GEMM_FLOAT8_FEW_ROWS = 64  # up to here a product's weight is streamed past all 
 GEMM_FLOAT8_FEW_BYTES = 150e6
 # Up to here rows in bfloat16 become 8 bits inside the product.  Every workgroup does that for itself, some 0.4 microseconds for each of the blocks of
 # 128 columns that a wave has (8 waves); beyond 4,096 columns that is more than a launch in front.
+# Groups' rows as well: on the device (a graph of calls), inside and in front, 16 rows of 16 groups of 2048 x 1408 13.3 and 13.6, of 2816 x 2048 23.0
+# and 21.0 (a launch more is 8 for the host), 64 of 64 83 and 64, 16 of 8 of 28672 x 4096 190 and 166, 8 of 8 of 4096 x 14336 93 and 82.
 GEMM_FLOAT8_INLINE_ROWS = 16
 GEMM_FLOAT8_INLINE_COLUMNS = 4096
+# Rows a group in the mean up to which groups go by the kernel of few rows, which walks a group's sixteens one behind another and reads the weight for each;
+# beyond it by tiles.  It knows the mean, not the largest.  Microseconds on the device, few and tiles, gated to 8 bits, shared out evenly / by shares
+# that fall with the 1.5th power / all to one group.  64 groups of 2816 x 2048: 4 in the mean 76 and 85 / 51 and 61 / 65 and 37, 8 80 and 86 / 73 and 71 /
+# 122 and 39, 16 89 and 105 / 119 and 97 / 236 and 57; 16 of them: 8 26 and 25 / 27 and 25 / 36 and 20, 16 29 and 25 / 38 and 25 / 65 and 21;
+# 8 of 28672 x 4096: 8 181 and 198 / 196 and 198 / 113 and 118, 16 211 and 202 / 281 and 201 / 216 and 126.
+GEMM_FLOAT8_FEW_IN_MEAN = 8
 GEMM_FLOAT8_SUMS_COLUMNS = 1024  # from here on gated rows in 8 bits of many rows may come of sums (a second launch is longer than the few blocks of a tile)
 _E4M3, _E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 
@@ -3293,7 +3301,7 @@ def _float8_product(out, x, w: Float8, bias, swiglu: bool, limit, gelu: bool, ex
     index = _gpu(*tensors)
     if m == 0:
         return out
-    few = m <= GEMM_FLOAT8_INLINE_ROWS * groups if grouped else m <= GEMM_FLOAT8_FEW_ROWS and (m <= 16 or n * columns < GEMM_FLOAT8_FEW_BYTES)
+    few = m <= GEMM_FLOAT8_FEW_IN_MEAN * groups if grouped else m <= GEMM_FLOAT8_FEW_ROWS and (m <= 16 or n * columns < GEMM_FLOAT8_FEW_BYTES)
     exact = bool(exact) and epilogue != 1  # (results in 32 bits always are)
     if exact and not grouped and m > 16 and cs is None:
         few = False  # (the stream's results in bfloat16 of more rows are of 8-bit products)
@@ -3307,7 +3315,7 @@ def _float8_product(out, x, w: Float8, bias, swiglu: bool, limit, gelu: bool, ex
     inline, at_rows, at_xs, ldxs = False, rows.data_ptr(), None if xs is None else xs.data_ptr(), 0 if xs is None else xs.stride(0)
     if xs is None:
         inline = (few and rows.dtype is torch.bfloat16 and columns % 8 == 0 and ldx < 1 << 23 and at_rows % 16 == 0 and (m == 1 or ldx % 8 == 0)
-                  and (grouped or (m <= GEMM_FLOAT8_INLINE_ROWS and columns <= GEMM_FLOAT8_INLINE_COLUMNS)))
+                  and m <= GEMM_FLOAT8_INLINE_ROWS and columns <= GEMM_FLOAT8_INLINE_COLUMNS)
         if not inline:
             # (as rows_float8 makes them: values and scales in one room)
             k8, ldxs = w.values.shape[-1], w.scale.shape[-1]
@@ -3348,7 +3356,7 @@ def gemm_float8(out, x, w: Float8, bias: torch.Tensor | None = None, *, swiglu: 
                 exact: bool = False):
     """The product of rows and a weight in 8 bits, sums in 32-bit over all of K, rounded once.  (Beyond 16 rows a bfloat16 result, and beyond 64, or
     16 of a weight of more than 150 MB, one in 8 bits, is that of the matrix cores' 8-bit products, whose sums of 16 are off by up to 2^-13 of the
-    largest product; a float32 result is not.  Of `grouped_float8` both are, beyond 16 rows a group in the mean.  With `exact` none is: sums of exact
+    largest product; a float32 result is not.  Of `grouped_float8` both are, beyond 8 rows a group in the mean.  With `exact` none is: sums of exact
     products, which leave in float32 and are rounded by a launch behind: 2048 x 12288 x 4096 takes 218 microseconds and not 91, 64 rows 22 and not 19.)
 
     x: `Float8` rows [M, K], or a bfloat16 or float32 matrix, which is taken to 8 bits as by rows_float8.

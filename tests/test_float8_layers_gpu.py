@@ -151,7 +151,7 @@ def test_every_product_of_a_model_with_biases(n, monkeypatch):
 @pytest.mark.parametrize("name", ["milozen-tiny", "nolavik-tiny", "felavik-tiny", "zotunex-tiny"])
 @pytest.mark.parametrize("n", [1, 30, 90])
 def test_every_product_of_experts(name, n, monkeypatch):
-    """Rows of the step's tokens, sorted by expert; up to 16 pairs an expert in the mean the sums are of exact products.  Few pairs and many."""
+    """Rows of the step's tokens, sorted by expert; up to 8 pairs an expert in the mean the sums are of exact products.  Few pairs and many."""
     from llmserve.config.registry import preset
 
     config = copy.deepcopy(preset(name))
@@ -176,7 +176,7 @@ def test_every_product_of_experts(name, n, monkeypatch):
                 continue
             gate_up = unpaired(kept.w_gate_up[e], part.intermediate)
             wd, dd = (held(ops.Float8(t.values[e], t.scale[e], t.columns), v) for t, v in ((w, gate_up), (w2, down[e])))
-            few = pairs <= 16 * experts
+            few = pairs <= 8 * experts
             mine = ops.Float8(act.values[a:b], act.scale[a:b], act.columns)
             check_units(mine, x[a:b], wd, not few, options["limit"])
             check_product(out[a:b], ops.Float8(x2.values[a:b], x2.scale[a:b], x2.columns), dd, sixteens=False)

@@ -201,3 +201,39 @@ def test_units_in_8_bits_of_a_row_are_the_same_beside_any_others(inter, k):
     for m, out in outs.items():
         assert torch.equal(out.values.view(torch.uint8), outs[64].values[:m].view(torch.uint8)), m
         assert torch.equal(out.scale.view(torch.uint8), outs[64].scale[:m].view(torch.uint8)), m
+
+
+@pytest.mark.parametrize("pairs,k,given,kernels", [
+    (16, 640, "bfloat16", ["few"]), (17, 640, "bfloat16", ["rows", "few"]), (16, 4104, "bfloat16", ["rows", "few"]), (16, 640, "float8", ["few"]),
+    (64, 640, "float8", ["few"]), (65, 640, "float8", ["tiles"]), (65, 640, "bfloat16", ["rows", "tiles"])])
+def test_which_kernels_groups_take(pairs, k, given, kernels, monkeypatch):
+    """Eight groups: rows become 8 bits inside the product up to 16 of up to 4,096 columns, as one weight's do; tiles beyond eight rows a group in the mean."""
+    names = {"llms_rows_float8": "rows", "llms_gemm_float8_few": "few", "llms_gemm_float8": "tiles"}
+    taken, real = [], ops()._entry
+    w8 = ops().weight_float8(torch.randn(8, 64, k, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(DEV))
+    x = torch.randn(pairs, k, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).to(DEV)
+    x8 = ops().rows_float8(ops().empty_float8(pairs, k, DEV), x)
+    counts = [pairs - 3, 0, 1, 0, 0, 2, 0, 0]
+    monkeypatch.setattr(ops(), "_entry", lambda library, name, arguments: taken.append(names[name]) or real(library, name, arguments))
+    out = ops().grouped_float8(torch.empty(pairs, 64, device=DEV), x if given == "bfloat16" else x8, w8, segments_of(counts))
+    assert taken == kernels
+    assert torch.equal(out, ops().grouped_float8(torch.empty(pairs, 64, device=DEV), x8, w8, segments_of(counts)))
+
+
+@pytest.mark.parametrize("counts", [[0] * 20 + [400] + [0] * 40 + [3, 90, 7], [1] * 30 + [130] + [1] * 33, [0, 0, 511, 1] + [0] * 60])
+@pytest.mark.parametrize("kind", ["rows", "float32"])
+def test_uneven_groups_of_few_rows_in_the_mean(counts, kind):
+    """One group far above the mean beside empty ones and ones of a row: as many sixteens as it has, one behind another."""
+    groups, inter, k = len(counts), 40, 300
+    pairs = sum(counts)
+    assert pairs <= 8 * groups
+    x8, w8, xd, wd = operands(pairs, 2 * inter, k, pairs, groups)
+    group = torch.repeat_interleave(torch.arange(groups), torch.tensor(counts))
+    y, off = torch.zeros(pairs, 2 * inter, dtype=torch.float64), torch.zeros(pairs, 2 * inter, dtype=torch.float64)
+    for g in set(group.tolist()):
+        y[group == g], off[group == g] = sums_of(xd[group == g], wd[g])
+    if kind == "float32":
+        out = ops().grouped_float8(torch.full((pairs, 2 * inter), float("nan"), device=DEV), x8, w8, segments_of(counts))
+        assert ((out.cpu().double() - y).abs() <= off).all()
+    else:
+        check_steps(ops().grouped_float8(ops().empty_float8(pairs, inter, DEV), x8, w8, segments_of(counts), swiglu=True), *units_of(y, off, inter))
