@@ -14,8 +14,8 @@
 //
 // 8192 x 8192 x 8192 takes 400 microseconds, 2750 TFLOP/s, on four waves, which read LDS for half as many bytes a product as eight (433; with 256
 // accumulators a lane in a register file of their own); 8192 x 57344 x 8192 2730, 2820 TFLOP/s; 2048 x 12288 x 4096 86 in tiles of 256 x 192.  The matrix
-// instructions alone would take 220; without the loads of X and W it is 308.  The clock is at 1.7 GHz of 2.4 then: what the card draws bounds it, and next
-// to that the L2.
+// instructions alone would take 220; without the loads of X and W it is 308.  The clock is at 1.76 GHz of 2.4 then, with the matrix
+// instructions at work in 77 % of the cycles (524,000 of 682,000 at 8192 cubed): what the card draws bounds it, and next to that the L2.
 //
 // Few tiles of a long K are shared out in parts of K, whose sums a second kernel adds up in their order: 200 x 4096 x 14336 58 -> 30 microseconds.
 //
