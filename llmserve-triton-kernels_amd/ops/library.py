@@ -3281,6 +3281,8 @@ def _float8_product(out, x, w: Float8, bias, swiglu: bool, limit, gelu: bool, ex
         if rows_out != m or cols_out != n_out:
             raise ValueError(f"out shape {tuple(out.shape)} is not {(m, n_out)}")
         c, cs, epilogue = out, None, 2 if swiglu else int(dtype is torch.float32)
+    if m and c.data_ptr() == rows.data_ptr():
+        raise ValueError("out may not lie on x, which other workgroups still read")
     tensors = [c, rows, w.values, w.scale]
     if bias is not None:
         if bias.dtype is not torch.bfloat16 or bias.shape != (n,) or not bias.is_contiguous():
@@ -3362,7 +3364,8 @@ def gemm_float8(out, x, w: Float8, bias: torch.Tensor | None = None, *, swiglu: 
     x: `Float8` rows [M, K], or a bfloat16 or float32 matrix, which is taken to 8 bits as by rows_float8.
     plain:   out[M, N] = x w^T (+ bias, bfloat16), bfloat16 or float32.
     swiglu:  w = [gate; up] ([2I, K]): out[M, I] = silu(gate) * up, or with `limit` or `gelu` the units of `silu_mul`, in 32-bit; out is
-             bfloat16, or a `Float8` (rows in 8 bits for the next product)."""
+             bfloat16, or a `Float8` (rows in 8 bits for the next product).
+    out shares no memory with x, w and bias."""
     return _float8_product(out, x, w, bias, swiglu, limit, gelu, exact, None, "gemm_float8")
 
 

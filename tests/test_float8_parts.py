@@ -145,3 +145,18 @@ def test_weights_beyond_32_bit_offsets_are_refused(n, k):
                    torch.empty((-(-n // 128), ops.float8_scale_columns(k)), dtype=torch.float8_e8m0fnu, device="meta"), k)
     with pytest.raises(ValueError, match="too large"):
         ops.gemm_float8(torch.empty((1, n), dtype=torch.float32, device="meta"), torch.empty((1, k), dtype=BF16, device="meta"), w)
+
+
+def test_a_result_on_its_own_rows_is_refused():
+    """Workgroups store theirs while others read X."""
+    x8 = ops.empty_float8(4, 256, "cpu")
+    x8.values.view(torch.uint8).zero_()
+    w = ops.Float8(torch.zeros(512, 256).to(torch.float8_e4m3fn), torch.ones(4, 4).to(torch.float8_e8m0fnu), 256)
+    with pytest.raises(ValueError, match="lie on x"):
+        ops.gemm_float8(x8, x8, w, swiglu=True)
+    x = torch.zeros(4, 256, dtype=BF16)
+    with pytest.raises(ValueError, match="lie on x"):
+        ops.gemm_float8(x, x, w, swiglu=True)
+    with pytest.raises(ValueError, match="GPU tensors only"):  # (beside it in one matrix: not refused for that)
+        both = torch.zeros(4, 512, dtype=BF16)
+        ops.gemm_float8(both[:, 256:], both[:, :256], w, swiglu=True)
